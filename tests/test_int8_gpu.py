@@ -691,3 +691,21 @@ def test_product_where_the_form_changes(m, n, k) -> None:
     ops.gemm_int8(x, xs, w, ws, out)
     product_holds(x, xs, w, ws, out)
     ops.check_device_errors()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [32, 64, 192, 320, 520])
+@pytest.mark.parametrize("k", [16, 256])
+def test_product_of_more_rows_than_one_turn_of_tiles(dtype, n, k) -> None:
+    """More than 74 tiles of 256 rows: a pair of CTAs takes several tiles of the last columns one after the other, each with an odd
+    number of pieces of the result (of 32 or 64 columns) among these widths. Every element, several times over."""
+    m = 3 * 74 * 256 + 77
+    assert ops.int8_product_form(m, n, k)[0] == 256
+    x, xs, w, ws = product_inputs(m, n, k, seed=n + k)
+    out = torch.empty(m, n, dtype=dtype, device="cuda")
+    for _ in range(3):
+        out.fill_(math.nan)
+        ops.gemm_int8(x, xs, w, ws, out)
+        product_holds(x, xs, w, ws, out)
+    ops.check_device_errors()

@@ -356,12 +356,13 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
 // One warp's 32 rows of an accumulator, 256 columns, scaled and stored. A row of the accumulator is a lane's, so that a store
 // straight from the registers touches 32 lines of memory with 16 bytes each: 128 bytes of each row go through shared memory
 // instead (two pieces in turn, swizzled as the copy expects them, so that eight lanes cover all banks) and out by TMA, which
-// also leaves out what lies beyond M and N. Rows off the 16-byte grid are stored from there by the warp, an element a lane and a
-// row after the other.
+// also leaves out what lies beyond M and N. `turn` counts a warp's pieces over all its tiles: a tile at the right edge may have an
+// odd number of them, and the next tile's first piece is then the other one, not the one that may still be on its way out.
+// Rows off the 16-byte grid are stored from there by the warp, an element a lane and a row after the other.
 template <typename T>
 __device__ __forceinline__ void drain_int8_tile(uint32_t tmem_acc, int row0, int M, int N, int n0, T* __restrict__ out, bool by_copy,
-                                                const CUtensorMap* map_out, unsigned char* pieces, const float* __restrict__ x_scales,
-                                                const float* tile_scales) {
+                                                const CUtensorMap* map_out, unsigned char* pieces, uint32_t& turn,
+                                                const float* __restrict__ x_scales, const float* tile_scales) {
   constexpr int COLS = 128 / sizeof(T);      // of a piece
   const int lane = threadIdx.x & 31, row = row0 + lane;
   const float xs = row < M ? x_scales[row] : 0.f;
@@ -372,7 +373,7 @@ __device__ __forceinline__ void drain_int8_tile(uint32_t tmem_acc, int row0, int
     uint32_t r[COLS];
 #pragma unroll
     for (int j = 0; j < COLS; j += 32) tmem_ld_32_nowait(tmem_acc + (uint32_t)(c * COLS + j), r + j);
-    unsigned char* piece = pieces + (c & 1) * MR_PIECE;
+    unsigned char* piece = pieces + (turn++ & 1u) * MR_PIECE;
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // the piece before the last has been read
     __syncwarp();
     tmem_ld_wait();
@@ -534,6 +535,7 @@ __global__ void __launch_bounds__(MR_THREADS) gemm_int8_pair_kernel(const __grid
     const int quad = warp & 3;
     unsigned char* pieces = tiles + (size_t)STAGES * MR_STAGE + quad * (2 * MR_PIECE);
     int t = 0;
+    uint32_t turn = 0;
     for (int tile = pair; tile < num_tiles; tile += num_pairs, ++t) {
       const int b = t & 1;
       const int m0 = (tile % tiles_m) * PAIR_BM + (int)rank * MR_BM, n0 = (tile / tiles_m) * MR_BN;
@@ -546,7 +548,7 @@ __global__ void __launch_bounds__(MR_THREADS) gemm_int8_pair_kernel(const __grid
       }
       tc_fence_after();
       drain_int8_tile<T>(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * MR_BN), m0 + quad * 32, M, N, n0, out, by_copy, &map_out,
-                         pieces, x_scales, tile_scales[b]);
+                         pieces, turn, x_scales, tile_scales[b]);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * b);
