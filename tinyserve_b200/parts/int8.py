@@ -115,15 +115,18 @@ class Int8KVNeed(PagedNeed):
         return Int8KVCacheEntry(group, k, v, scales[0], scales[1], page_size)
 
 
-_rows: dict[torch.device, torch.Tensor] = {}
+_rows: dict[torch.device, list[torch.Tensor]] = {}
 
 
 def _row_numbers(device: torch.device, t: int) -> torch.Tensor:
-    """0, 1, 2, ... as int32: where each token's key and value lie in a scratch of one row per token."""
-    have = _rows.get(device)
-    if have is None or have.numel() < t:
-        have = _rows[device] = torch.arange(max(1 << 16, t), dtype=torch.int32, device=device)
-    return have[:t]
+    """0, 1, 2, ... as int32: where each token's key and value lie in a scratch of one row per token. Recorded steps of any model
+    hold the addresses of the numbers they were given, so numbers that were handed out are never let go of; new ones are at
+    least twice as many, so all of them together are no more than twice the last. (A step runs before it is recorded: none
+    are made inside a recording.)"""
+    made = _rows.setdefault(device, [])
+    if not made or made[-1].numel() < t:
+        made.append(torch.arange(max(t, 2 * made[-1].numel() if made else 1 << 16), dtype=torch.int32, device=device))
+    return made[-1][:t]
 
 
 class Int8GQAAttention(GQAAttention):
