@@ -709,3 +709,17 @@ def test_product_of_more_rows_than_one_turn_of_tiles(dtype, n, k) -> None:
         ops.gemm_int8(x, xs, w, ws, out)
         product_holds(x, xs, w, ws, out)
     ops.check_device_errors()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [16, 20, 37, 300, 301])
+def test_values_of_no_items_at_all(dtype, width) -> None:
+    """Every item asked for lies outside: NaN, in each of the readers' forms (vectors of 16 and 4, single codes, long groups)."""
+    rows = torch.tensor([0, -1, 5], dtype=torch.int32, device="cuda")
+    out = torch.zeros(3, width, dtype=dtype, device="cuda")
+    ops.int8_values(torch.empty(0, width, dtype=torch.int8, device="cuda"), torch.empty(0, device="cuda"), out, rows=rows)
+    assert bool(torch.isnan(out).all())
+    out = torch.zeros(3, 2, 5, width, dtype=dtype, device="cuda")
+    ops.int8_values(torch.empty(0, 2, 5, width, dtype=torch.int8, device="cuda"), torch.empty(0, 2, device="cuda"), out, rows=rows)
+    assert bool(torch.isnan(out).all())

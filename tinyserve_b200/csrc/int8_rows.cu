@@ -363,15 +363,18 @@ __global__ void __launch_bounds__(256) int8_values_kernel(const int8_t* __restri
   const size_t group = (size_t)(there ? from : 0) * heads + (to - i * heads);
   const float s = there ? scales[group] : __uint_as_float(INT8_NAN_BITS);
   const int8_t* p = codes + group * in_width + c;
+  // (nothing is read for an item outside: there may be no codes at all)
   if constexpr (VEC == 1) {
-    out[at] = from_float<T>((float)p[0] * s);
+    out[at] = from_float<T>((there ? (float)p[0] : 0.f) * s);
   } else {
-    uint32_t w[VEC / 4];
-    if constexpr (VEC == 16) {
-      const uint4 x = *reinterpret_cast<const uint4*>(p);
-      w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-    } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    uint32_t w[VEC / 4] = {};
+    if (there) {
+      if constexpr (VEC == 16) {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+      } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+      }
     }
     float f[VEC];
 #pragma unroll
@@ -408,7 +411,7 @@ __global__ void __launch_bounds__(256) int8_long_values_kernel(const int8_t* __r
   T* o = out + (size_t)to * out_width;
   float f[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) f[e] = c0 + 256 * e < out_width ? (float)p[c0 + 256 * e] : 0.f;
+  for (int e = 0; e < 4; ++e) f[e] = there && c0 + 256 * e < out_width ? (float)p[c0 + 256 * e] : 0.f;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (c0 + 256 * e < out_width) o[c0 + 256 * e] = from_float<T>(f[e] * s);
