@@ -536,6 +536,15 @@ def test_what_the_cache_refuses() -> None:
     refuses("head size", ops.paged_attention_int8, f(3, 4, 512), *big, 1.0, 0, f(3, 2048))
 
 
+def test_attention_refuses_rows_that_are_not_the_steps() -> None:
+    """The kernels find a request's rows by the step's lengths: fewer rows than the step has tokens would be read behind their end."""
+    ctx = SimpleNamespace(num_tokens=3, num_seqs=2, max_query_len=2, num_prefill=1, num_decode=1, max_context_len=40)
+    cache = (*(torch.empty(9, 2, 16, 64, dtype=torch.int8) for _ in range(2)), torch.empty(9, 2), torch.empty(9, 2))
+    tables = torch.zeros(2, 4, dtype=torch.int32)
+    for t in (0, 2, 4):
+        refuses("row per token", ops.paged_attention_int8, torch.empty(t, 4, 64), *cache, 16, tables, ctx, 1.0, 0, torch.empty(t, 256))
+
+
 @gpu
 def test_what_the_kernels_refuse_of_tensors() -> None:
     """Types, layouts and addresses that only a tensor on the device shows."""

@@ -2685,6 +2685,8 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     hkv = k_cache.shape[1]
     dt = q.dtype
     pages = _int8_cache("paged_attention_int8", k_cache, v_cache, k_scales, v_scales, page_size, hkv, d, block_tables, ctx)
+    if t != ctx.num_tokens:
+        raise KernelError("paged_attention_int8: q must have a row per token of the step")
     if out.dtype != dt or out.numel() != t * hq * d or hq % hkv or window < 0 or not scale > 0:
         raise KernelError("paged_attention_int8: out shape or dtype, head grouping, window or scale (a positive number)")
     if d > 256:
