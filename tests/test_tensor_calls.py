@@ -67,6 +67,21 @@ def test_words_and_refusals(module) -> None:
         call(None, 1 << 70, 0, 0.0, 0, 0)
 
 
+def test_sizes_beyond_32_bits_are_refused(monkeypatch) -> None:
+    """Where the host module does not take a call it is made through ctypes, which would cut such a size off without a word."""
+    made = []
+    monkeypatch.setattr(ops, "_dev", lambda t, name, dtype=None: 16)
+    monkeypatch.setattr(ops, "_fn", lambda name: lambda *words: made.append(words) or 0)
+    x, codes, scales = torch.zeros(1), torch.zeros(1, dtype=torch.int8), torch.zeros(1)
+    call = ops._TensorCall("ts_act_mul_int8", "act_mul_int8", "d8fnnnn=p", "x out scales")
+    for sizes in ((2 ** 31, 64, 64, 3), (5, 64, 2 ** 32 + 64, 3), (-2 ** 31 - 1, 64, 64, 3)):
+        with pytest.raises(ops.KernelError, match="act_mul_int8: .* 32 bits"):
+            call._by_ctypes((x, codes, scales, *sizes, 0))
+    assert not made
+    call._by_ctypes((x, codes, scales, 2 ** 31 - 1, 64, 64, 3, 2 ** 48))       # an address may be as large as it is
+    assert len(made) == 1 and made[0][3] == 2 ** 31 - 1 and made[0][-1] == 2 ** 48
+
+
 @pytest.mark.gpu
 def test_only_what_fits_is_taken(module) -> None:
     at = ctypes.cast(take, ctypes.c_void_p).value

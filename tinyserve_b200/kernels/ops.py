@@ -2467,6 +2467,8 @@ class _TensorCall:
                 continue
             a = next(rest)
             if what in "nxp":
+                if what == "n" and _SIGNATURES[self.name][len(words)] is _i and not -2 ** 31 <= a < 2 ** 31:
+                    raise KernelError(f"{self.what}: a size of {a} is beyond 32 bits")      # (ctypes would cut it off)
                 words.append(a)
                 continue
             name = next(names)
