@@ -38,6 +38,22 @@ def test_patterns_fit_the_entry_points(module) -> None:
     assert lib.ts_list_function(b"ts_no_such_function", ctypes.addressof(kinds)) is None
 
 
+def test_without_a_compiler_or_the_cuda_headers_calls_go_through_ctypes(monkeypatch, tmp_path) -> None:
+    """A machine that has the built library and no toolkit, or no g++: no module, and no error."""
+    def none() -> str:
+        raise build.KernelBuildError("nvcc not found")
+
+    with monkeypatch.context() as m:
+        m.setattr(build, "find_nvcc", none)
+        assert build.build_calls(tmp_path) is None
+        m.setattr(build, "_calls", [])
+        m.setattr(build, "build_dir", lambda: tmp_path)
+        assert build.calls() is None
+    monkeypatch.setenv("PATH", str(tmp_path))
+    assert build.build_calls(tmp_path) is None
+    assert not list(tmp_path.iterdir())
+
+
 SEEN: list[int] = []
 WORDS = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.POINTER(ctypes.c_uint64))
 

@@ -185,7 +185,11 @@ def build_calls(out_dir: Path) -> Path | None:
                 return target
         except (OSError, ValueError):
             pass
-    cuda = Path(find_nvcc()).parent.parent
+    try:
+        cuda = Path(find_nvcc()).parent.parent
+    except KernelBuildError as e:
+        _say(f"no host module ({e}): calls go through ctypes")
+        return None
     tmp = out_dir / f".{CALLS_NAME}.{os.getpid()}.so"
     cmd = ["g++", *flags, f"-I{root / 'include'}", f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
            f"-I{sysconfig.get_paths()['include']}", f"-I{cuda / 'include'}", str(src), "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-lc10"]
