@@ -3,7 +3,7 @@
 The model reports, per cache user (a call of its run order and a mixer of that call's block),
 what it keeps between steps: a ``PagedNeed``, a ``SlotNeed`` or nothing (``parts.base``). The
 manager serves the two families through their own methods (``allocate``, ``entry``,
-``bytes_per_token``), so a need of a new shape is a new subclass and no change here.
+``bytes_per_page``), so a need of a new shape is a new subclass and no change here.
 
 Users with equal paged needs share a **page group**: one pool of pages, one allocator and, per
 request, one block table. Groups with different needs (all positions, a window of them, another
@@ -60,7 +60,7 @@ class PageGroup:
         return self.num_pages
 
     def bytes_per_page(self, element_size: int) -> int:
-        return len(self.calls) * self.need.bytes_per_token(element_size) * self.page_size
+        return len(self.calls) * self.need.bytes_per_page(element_size, self.page_size)
 
     def most_pages_of(self, num_tokens: int, step_tokens: int) -> int:
         """The most pages of this group that a request of up to ``num_tokens`` tokens ever holds
@@ -186,6 +186,11 @@ class CacheManager:
     @staticmethod
     def bytes_per_token(needs: Sequence[CacheNeed | None], element_size: int) -> int:
         return sum(n.bytes_per_token(element_size) for n in needs if isinstance(n, PagedNeed))
+
+    @staticmethod
+    def bytes_per_page(needs: Sequence[CacheNeed | None], element_size: int, page_size: int) -> int:
+        """What one page more in every pool takes."""
+        return sum(n.bytes_per_page(element_size, page_size) for n in needs if isinstance(n, PagedNeed))
 
     @property
     def utilization(self) -> float:

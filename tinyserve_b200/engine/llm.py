@@ -42,7 +42,7 @@ class LLM:
         needs = model.cache_needs()
         if num_pages is None:
             elem = torch.empty(0, dtype=model.dtype).element_size()
-            per_page = CacheManager.bytes_per_token(needs, elem) * page_size
+            per_page = CacheManager.bytes_per_page(needs, elem, page_size)
             if model.device.type == "cuda":
                 free, _ = torch.cuda.mem_get_info(model.device)
             else:

@@ -91,6 +91,10 @@ class PagedNeed(CacheNeed):
     def bytes_per_token(self, element_size: int) -> int:
         raise NotImplementedError
 
+    def bytes_per_page(self, element_size: int, page_size: int) -> int:
+        """What a page of one call takes, with all that belongs to the page and not to its tokens."""
+        return self.bytes_per_token(element_size) * page_size
+
     def allocate(self, num_calls: int, num_pages: int, page_size: int, dtype: torch.dtype,
                  device: torch.device) -> torch.Tensor:
         """The storage of a whole group: ``num_pages`` already counts the pad page (the last one,

@@ -95,16 +95,16 @@ class Int8KVNeed(PagedNeed):
     window: int | None = None
 
     def bytes_per_token(self, element_size: int) -> int:
-        # the scales of a page are 8 bytes a head: with pages of 8 tokens and more, one byte a token and head at most
+        # the scales of a page are 8 bytes a head: one byte a token and head with pages of 8 tokens (``bytes_per_page`` is exact)
         return self.num_kv_heads * (2 * self.head_dim + 1)
 
-    def _page_bytes(self, page_size: int) -> int:
+    def bytes_per_page(self, element_size: int, page_size: int) -> int:
         return 2 * self.num_kv_heads * page_size * self.head_dim + -(-2 * self.num_kv_heads * 4 // 16) * 16      # (calls start on 16 bytes)
 
     def allocate(self, num_calls, num_pages, page_size, dtype, device):
         if page_size * self.head_dim % 16:
             raise ValueError(f"pages of {page_size} tokens with heads of {self.head_dim}: 8-bit pages lie on 16 bytes")
-        return torch.zeros((num_calls, num_pages, self._page_bytes(page_size)), dtype=torch.int8, device=device)
+        return torch.zeros((num_calls, num_pages, self.bytes_per_page(1, page_size)), dtype=torch.int8, device=device)
 
     def entry(self, storage, call_in_group, group, page_size):
         num_pages, heads = storage.shape[1], self.num_kv_heads
