@@ -732,3 +732,60 @@ def test_values_of_no_items_at_all(dtype, width) -> None:
     out = torch.zeros(3, 2, 5, width, dtype=dtype, device="cuda")
     ops.int8_values(torch.empty(0, 2, 5, width, dtype=torch.int8, device="cuda"), torch.empty(0, 2, device="cuda"), out, rows=rows)
     assert bool(torch.isnan(out).all())
+
+
+def portions_case(new, lens, hq, hkv, d, page, dtype, window=0, seed=0):
+    ctx = step_of(new, lens, dtype)
+    tables, pages = tables_for(lens, page)
+    cache = cache_of(pages, hkv, page, d, seed=seed)
+    quiet_elsewhere(cache, tables, lens, page, new, window)
+    return ctx, tables, cache, rnd(sum(new), hq, d, dtype=dtype, seed=6)
+
+
+@gpu
+def test_portions_take_no_more_scratch_than_they_may() -> None:
+    """Pages of all requests of the step, as values, would be 1.3 GB here; a second layer works in the memory of the first."""
+    ctx, tables, cache, q = portions_case([32, 1] * 40, [8192, 9] * 40, 32, 8, 128, 16, torch.bfloat16)
+    for _ in range(2):
+        ctx.arena.next_frame()
+        out = attend(q, cache, 16, tables, ctx, 0, 0.09)
+    assert ctx.arena.reserved_bytes <= (512 << 20) + (1 << 20)
+    attention_holds(q, cache, 16, tables, ctx, 0, out, 0.09)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d,page", [(8, 2, 128, 16), (4, 4, 64, 16), (6, 2, 80, 16), (12, 2, 96, 32), (3, 1, 36, 5), (4, 2, 256, 24)])
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("pages_at_once", [0, 20, 60, 100])
+def test_portions_with_little_scratch(dtype, hq, hkv, d, page, window, pages_at_once, monkeypatch) -> None:
+    """Some requests at a time, beside single tokens between them; requests that alone are beyond the scratch go over the codes."""
+    new = [200, 1, 31, 2, 1, 300, 90, 1, 64]
+    lens = [20 * page, 30, 33 * page - 1 if page > 1 else 40, 2, 700, 59 * page, 19 * page, 1, 90 * page]
+    new = [min(a, b) for a, b in zip(new, lens)]
+    ctx, tables, cache, q = portions_case(new, lens, hq, hkv, d, page, dtype, window)
+    monkeypatch.setattr(ops, "_int8_direct_rows", lambda *_: 0)
+    limit = pages_at_once * 2 * hkv * page * d * q.element_size()
+    monkeypatch.setattr(ops, "INT8_PORTIONS_SCRATCH_BYTES", limit)
+    out = attend(q, cache, page, tables, ctx, window, d ** -0.5)
+    attention_holds(q, cache, page, tables, ctx, window, out, d ** -0.5)
+    assert (ctx.arena.reserved_bytes > 0) == (pages_at_once > 0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_portions_without_memory_for_scratch(dtype, monkeypatch) -> None:
+    """They go over the codes; the arena is as it was."""
+    new, lens = [100, 1, 300], [1000, 40, 2000]
+    ctx, tables, cache, q = portions_case(new, lens, 8, 2, 128, 16, dtype)
+    monkeypatch.setattr(ops, "_int8_direct_rows", lambda *_: 0)
+    lost = []
+
+    def take(self, nbytes):
+        lost.append(nbytes)
+        raise torch.cuda.OutOfMemoryError("no memory")
+
+    monkeypatch.setattr(Arena, "take_for_call", take)
+    out = attend(q, cache, 16, tables, ctx, 0, 0.09)
+    assert len(lost) == 1 and lost[0] >= 3000 * 2 * 2 * 128 * q.element_size()
+    attention_holds(q, cache, 16, tables, ctx, 0, out, 0.09)

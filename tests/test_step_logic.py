@@ -112,3 +112,31 @@ def test_an_arena_that_finds_no_memory_asks_for_none_of_it_later(monkeypatch) ->
         b = arena.take((1000,), torch.float32)
         assert a.data_ptr() + 4000 <= b.data_ptr() or b.data_ptr() + 4000 <= a.data_ptr()
     assert arena.reserved_bytes < 1 << 20
+
+
+def test_memory_for_a_call_is_one_buffer_of_what_is_asked_for(monkeypatch) -> None:
+    """No frames, no doubling; the old buffer is gone before the larger one is made, and after a failure there is none."""
+    from tinyserve_b200.engine import arena as module
+
+    arena = module.Arena("cpu")
+    a = arena.take_for_call(5000)
+    assert a.numel() == 5000 and a.dtype == torch.uint8 and arena.reserved_bytes == 5000
+    at, moves = a.data_ptr(), arena.moves
+    arena.begin_step()
+    arena.next_frame()
+    b = arena.take_for_call(4000)
+    assert b.data_ptr() == at and arena.reserved_bytes == 5000 and arena.moves == moves
+    assert arena.take_for_call(5001).numel() == 5001 and arena.reserved_bytes == 5001 and arena.moves == moves + 1
+    empty, held = torch.empty, []
+
+    def limited(*shape, **kw):
+        held.append(arena.reserved_bytes)
+        if shape[0] > 1 << 20:
+            raise torch.cuda.OutOfMemoryError("no memory")
+        return empty(*shape, **kw)
+
+    monkeypatch.setattr(module.torch, "empty", limited)
+    with pytest.raises(torch.cuda.OutOfMemoryError):
+        arena.take_for_call(1 << 21)
+    assert held[-1] == 0 and arena.reserved_bytes == 0
+    assert arena.take_for_call(100).numel() == 100

@@ -5,6 +5,8 @@ tables, logits); two ``frames`` alternate from layer to layer, so that the outpu
 leaves pending on the residual stream is still intact while the next layer, working in the
 other frame, reads it. Nothing is allocated from the device allocator in steady state; a
 region grows (once, outside any graph capture) when a step needs more than it has.
+Beside them lies one buffer for what is large and lives for a single call (``take_for_call``):
+every call of that kind works in the same memory, one after the other on the step's stream.
 
 The layers of a step ask for the same shapes at the same offsets, so a region keeps the views it
 has made of its buffer (slicing and viewing took a quarter of the host's time for a step that is
@@ -100,6 +102,8 @@ class Arena:
         self._frames = (_Region(self.device), _Region(self.device))
         self._current = self._step
         self._frame_index = 0
+        self._for_call = torch.empty(0, dtype=torch.uint8, device=self.device)
+        self._call_moves = 0
 
     def begin_step(self) -> None:
         self._step.reset()
@@ -134,11 +138,20 @@ class Arena:
     def take_step(self, shape: tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
         return self._step.take(tuple(shape), dtype)
 
+    def take_for_call(self, nbytes: int) -> torch.Tensor:
+        """``nbytes`` bytes (uint8) until the next call of this method: no larger than the largest taken so far, and the old buffer
+        goes before a larger one is made."""
+        if nbytes > self._for_call.numel():
+            self._for_call = torch.empty(0, dtype=torch.uint8, device=self.device)
+            self._call_moves += 1
+            self._for_call = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        return self._for_call[:nbytes]
+
     @property
     def moves(self) -> int:
         """Grows whenever a region's buffer is made anew (what was handed out before then lies elsewhere)."""
-        return self._step.moves + sum(f.moves for f in self._frames)
+        return self._step.moves + sum(f.moves for f in self._frames) + self._call_moves
 
     @property
     def reserved_bytes(self) -> int:
-        return self._step.buf.numel() + sum(f.buf.numel() for f in self._frames)
+        return self._step.buf.numel() + sum(f.buf.numel() for f in self._frames) + self._for_call.numel()

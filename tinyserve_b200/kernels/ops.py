@@ -2698,11 +2698,13 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     group, longest = hq // hkv, ctx.max_query_len
     num_prefill = ctx.num_prefill
     seen = min(ctx.max_context_len, window + longest) if window else ctx.max_context_len
-    if num_prefill and num_prefill * hq * longest > _int8_direct_rows(dt, d, page_size, seen):
-        _portions_int8(q, k_cache, v_cache, k_scales, v_scales, page_size, block_tables, ctx, scale, window, out)
-        num_prefill = 0
     tensor_cores = d in (64, 96, 128) and page_size % 8 == 0
-    for seqs, count, queries in ((ctx.decode_seqs, ctx.num_decode, 1), (ctx.prefill_seqs, num_prefill, longest)):
+    over_codes = [(0, num_prefill)]          # of the portions, from which to which
+    if num_prefill and num_prefill * hq * longest > _int8_direct_rows(dt, d, page_size, seen):
+        # (a launch over the codes takes 65,535 tiles of rows and heads at most)
+        most = 65535 // hkv * (16 if tensor_cores and dt == torch.bfloat16 else 8) // group
+        over_codes = _portions_int8(q, k_cache, v_cache, k_scales, v_scales, page_size, block_tables, ctx, scale, window, out, longest <= most)
+    for seqs, count, queries in ((ctx.decode_seqs, ctx.num_decode, 1), *((ctx.prefill_seqs[a: b], b - a, longest) for a, b in over_codes)):
         if count:
             keys = min(ctx.max_context_len, window + queries) if window else ctx.max_context_len
             _attention_int8(q, out, k_cache, v_cache, k_scales, v_scales, block_tables, block_tables.shape[1], ctx.cu_query_lens,
@@ -2767,26 +2769,63 @@ def int8_attention_form(groups: int, rows: int, keys: int, tensor_cores: bool, d
     return tile, max(1, splits), 4
 
 
+# Keys and values of pages that portions look at, as values: the most bytes that an arena holds for them (a recorded portion has
+# an arena of its own).
+INT8_PORTIONS_SCRATCH_BYTES = 512 << 20
+
+
 def _portions_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
-                   page_size: int, block_tables: torch.Tensor, ctx: Any, scale: float, window: int, out: torch.Tensor) -> None:
-    """The prompt portions of a step over an 8-bit cache: the pages they look at become values in scratch of the arena, once,
-    and :func:`paged_attention` reads those."""
+                   page_size: int, block_tables: torch.Tensor, ctx: Any, scale: float, window: int, out: torch.Tensor,
+                   codes_can: bool) -> "list[tuple[int, int]]":
+    """The prompt portions of a step over an 8-bit cache: the pages they look at become values in memory of the arena, once,
+    and :func:`paged_attention` reads those; as many requests at a time as it may hold. Returns which portions (of
+    ``ctx.prefill_seqs``, from which to which) are left to go over the codes, which needs no scratch: requests that alone are beyond
+    it, or all where there is no memory for it. ``codes_can``: the kernel over the codes takes portions of this length."""
     hkv, d, dt = k_cache.shape[1], q.shape[2], q.dtype
-    if ctx.recorded or getattr(ctx, "context_lens", None) is None:      # (a recording replays longer contexts than it was made with)
-        pages = ctx.num_prefill * -(-ctx.max_context_len // page_size)
-    else:
-        pages = sum(-(-n // page_size) for n, new in zip(ctx.context_lens, ctx.query_lens) if new > 1)
-    pages = 1 << (pages - 1).bit_length()        # few sizes: descriptors of cache tensors are kept by place and size
     width = -(-ctx.max_context_len // page_size)
-    k, v = (ctx.arena.take((pages, hkv, page_size, d), dt) for _ in range(2))
+    most = INT8_PORTIONS_SCRATCH_BYTES // (2 * hkv * page_size * d * q.element_size())
+    if ctx.recorded or getattr(ctx, "context_lens", None) is None:      # (a recording replays longer contexts than it was made with)
+        runs, requests = [(0, ctx.num_prefill, ctx.num_prefill * width)], None
+    else:
+        requests = [i for i, new in enumerate(ctx.query_lens) if new > 1]
+        runs = []
+        for i, r in enumerate(requests):
+            pages = -(-ctx.context_lens[r] // page_size)
+            if runs and runs[-1][2] + pages <= most:
+                runs[-1] = (runs[-1][0], i + 1, runs[-1][2] + pages)
+            else:
+                runs.append((i, i + 1, pages))
+    left = [(a, b) for a, b, pages in runs if pages > most and codes_can]
+    runs = [run for run in runs if run[2] <= most or not codes_can]
+    if not runs:
+        return left
+    pages = max(pages for _, _, pages in runs)
+    pages = max(pages, min(most, 1 << (pages - 1).bit_length()))        # few sizes: descriptors of cache tensors are kept by place and size
+    size = pages * hkv * page_size * d * q.element_size()
+    second = -(-size // 256) * 256                                       # (both begin on the grid of the arena)
+    try:
+        both = ctx.arena.take_for_call(second + size)
+    except torch.cuda.OutOfMemoryError:
+        if not codes_can:
+            raise
+        return left + [(a, b) for a, b, _ in runs]
+    k, v = (both[at: at + size].view(dt).view(pages, hkv, page_size, d) for at in (0, second))
     tables = ctx.arena.take((ctx.num_seqs, width), torch.int32)
-    _kv_values_int8(k_cache, v_cache, k_scales, v_scales, block_tables, block_tables.shape[1], ctx.cu_query_lens, ctx.context_lens_dev,
-                    k, v, tables, width, pages, ctx.num_seqs, hkv, d, page_size, k_cache.shape[0], window, _stream())
-    paged_attention(q, k, v, page_size, tables, _PortionsOnly(ctx), scale, window, out)
+    for a, b, _ in runs:
+        part, lo, hi = _PortionsOnly(ctx), 0, ctx.num_seqs
+        if b - a < ctx.num_prefill:
+            lo, hi = requests[a], requests[b - 1] + 1
+            part.prefill_seqs, part.num_prefill = ctx.prefill_seqs[a: b], b - a
+            part.query_lens, part.context_lens = ([of[r] for r in requests[a: b]] for of in (ctx.query_lens, ctx.context_lens))
+        _kv_values_int8(k_cache, v_cache, k_scales, v_scales, block_tables[lo: hi], block_tables.shape[1], ctx.cu_query_lens[lo: hi + 1],
+                        ctx.context_lens_dev[lo: hi], k, v, tables[lo: hi], width, pages, hi - lo, hkv, d, page_size, k_cache.shape[0],
+                        window, _stream())
+        paged_attention(q, k, v, page_size, tables, part, scale, window, out)
+    return left
 
 
 class _PortionsOnly:
-    """A step's context without its single tokens."""
+    """A step's context without its single tokens (and with what is set on it instead of the step's)."""
 
     num_decode = 0
 
