@@ -342,7 +342,9 @@ def build_parts(spec: ModelSpec) -> ModelParts:
 
 class DecoderModel:
     """Parts with weights on a device, in one dtype, ready to run steps. ``eight_bit``: the layers' projections and the cache of
-    keys and values are held in 8 bits (``parts.int8``), made from the given weights, which are let go of."""
+    keys and values are held in 8 bits (``parts.int8``). ``from_folder`` and ``from_config`` make a weight's codes as soon as the
+    weight is there and let go of it before the next, so a model that only fits in 8 bits can be loaded; ``tensors`` given here
+    may hold the weights either way."""
 
     def __init__(self, config: ModelConfig, tensors: Mapping[str, torch.Tensor],
                  dtype: torch.dtype, device: torch.device | str, eight_bit: bool = False) -> None:

@@ -50,7 +50,8 @@ class TensorSpec:
     ``init`` names the law of the random-weights mode: ``"normal"`` is N(0, std),
     ``"one_plus_normal"`` is 1 + N(0, std). ``keep_32bit`` marks tensors that stay 32-bit
     when the checkpoint stores them so, whatever the run's dtype; integer tables are always
-    kept as int32.
+    kept as int32. ``becomes``: what the part keeps is made from the tensor by this function as soon as the
+    tensor is there, and bound in its place, so that the tensor itself can go before the next one comes.
     """
 
     name: str
@@ -61,6 +62,10 @@ class TensorSpec:
     merged_rows: tuple[int, ...] = ()
     keep_32bit: bool = False
     integer: bool = False
+    becomes: "Callable[[torch.Tensor], Any] | None" = None
+
+    def taken(self, tensor: torch.Tensor) -> Any:
+        return tensor if self.becomes is None else self.becomes(tensor)
 
 
 # ------------------------------------------------------------------------ cache needs

@@ -1,6 +1,6 @@
 """The parts of a pre-norm decoder layer in 8 bits: rows of the stream normed into 8-bit integers with a scale each, projections
 as products of such rows with 8-bit weights (a scale per output channel), keys and values cached as 8-bit integers with a scale
-per page and head. The weights are made from the checkpoint's when they are bound; everything between the products (norm,
+per page and head. The weights are made from the checkpoint's as they are loaded, one after the other; everything between the products (norm,
 rotation, softmax, activation, the residual stream) is in the model dtype or 32-bit as in the plain parts.
 
 ``eight_bit(spec)`` puts these parts in the place of a model's plain ones. Upstream has no counterpart.
@@ -16,7 +16,7 @@ import torch
 from ..config.base import ModelSpec, PartSpec, UnsupportedConfigError
 from ..kernels import ops
 from .attention import GQAAttention
-from .base import EVERY_STEP, PagedNeed, ResidualStream, StepContext, register_feed_forward, register_mixer, register_norm
+from .base import EVERY_STEP, PagedNeed, ResidualStream, StepContext, TensorSpec, register_feed_forward, register_mixer, register_norm
 from .mlp import SwiGLU
 from .norm import RMSNorm
 
@@ -43,12 +43,21 @@ class Int8Weight:
     def __init__(self, w: torch.Tensor) -> None:
         self.codes, self.scales = ops.int8_weight(w)
 
+    @classmethod
+    def of(cls, w: "torch.Tensor | Int8Weight") -> "Int8Weight":
+        """A weight as it was loaded: as codes already, or as the matrix they are made from."""
+        return w if isinstance(w, cls) else cls(w)
+
     def project(self, x: Int8Rows, ctx: StepContext, rows: int | None = None) -> torch.Tensor:
         """``x w^T`` in the model dtype; ``rows``: of the first so many rows of ``w`` only."""
         codes, scales = (self.codes, self.scales) if rows is None else (self.codes[:rows], self.scales[:rows])
         out = ctx.arena.take((x.num_rows, codes.shape[0]), ctx.dtype)
         ops.gemm_int8(x.codes, x.scales, codes, scales, out)
         return out
+
+
+def _projections_in_8_bits(specs: list[TensorSpec]) -> list[TensorSpec]:
+    return [replace(s, becomes=Int8Weight) if len(s.shape) == 2 else s for s in specs]
 
 
 class Int8RMSNorm(RMSNorm):
@@ -140,13 +149,16 @@ class Int8GQAAttention(GQAAttention):
     def cache_need(self) -> Int8KVNeed:
         return Int8KVNeed(self.num_kv_heads, self.head_dim, self.window)
 
-    def bind(self, prefix: str, tensors: Mapping[str, torch.Tensor]) -> None:
-        super().bind(prefix, tensors)
+    def tensor_specs(self, prefix: str) -> list[TensorSpec]:
+        return _projections_in_8_bits(super().tensor_specs(prefix))
+
+    def bind(self, prefix: str, tensors: "Mapping[str, torch.Tensor | Int8Weight]") -> None:
         p = prefix + self.prefix
-        self.qkv, self.o = Int8Weight(self.w_qkv), Int8Weight(self.w_o)
+        self.qkv, self.o = Int8Weight.of(tensors[p + "qkv_proj.weight"]), Int8Weight.of(tensors[p + "o_proj.weight"])
         self.eight_bit = {p + "qkv_proj.weight": self.qkv, p + "o_proj.weight": self.o}
-        _row_numbers(self.w_qkv.device, 1)
-        self.w_qkv = self.w_q = self.w_o = None
+        if self.qk_norm:
+            self.q_norm_w, self.k_norm_w = tensors[p + "q_norm.weight"], tensors[p + "k_norm.weight"]
+        _row_numbers(self.qkv.codes.device, 1)
 
     def forward(self, x: Int8Rows, ctx: StepContext, cache: Int8KVCacheEntry, writes_cache: bool, position: Any) -> torch.Tensor:
         t, h, hkv, d = x.num_rows, self.num_heads, self.num_kv_heads, self.head_dim
@@ -174,12 +186,13 @@ class Int8SwiGLU(SwiGLU):
     takes_lazy_input = False
     adds_to_stream = False
 
-    def bind(self, prefix: str, tensors: Mapping[str, torch.Tensor]) -> None:
-        super().bind(prefix, tensors)
+    def tensor_specs(self, prefix: str) -> list[TensorSpec]:
+        return _projections_in_8_bits(super().tensor_specs(prefix))
+
+    def bind(self, prefix: str, tensors: "Mapping[str, torch.Tensor | Int8Weight]") -> None:
         p = prefix + self.prefix
-        self.gate_up, self.down = Int8Weight(self.w_gate_up), Int8Weight(self.w_down)
+        self.gate_up, self.down = Int8Weight.of(tensors[p + "gate_up_proj.weight"]), Int8Weight.of(tensors[p + "down_proj.weight"])
         self.eight_bit = {p + "gate_up_proj.weight": self.gate_up, p + "down_proj.weight": self.down}
-        self.w_gate_up = self.w_down = None
 
     def streamed_weights(self) -> list[torch.Tensor]:
         return []

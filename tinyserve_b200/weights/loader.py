@@ -137,7 +137,7 @@ def load_tensors(model_dir: str | Path, specs: Iterable[TensorSpec], dtype: torc
                     row += part.shape[0]
             if t.dtype.is_floating_point and not bool(torch.isfinite(t).all()):
                 raise WeightLoadError(f"{name} has inf or nan after casting to {target}")
-            out[name] = t.contiguous()
+            out[name] = spec.taken(t.contiguous())
     finally:
         handles.clear()
     return out

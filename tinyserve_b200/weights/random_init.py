@@ -67,9 +67,9 @@ def random_bound_tensors(specs: Iterable[TensorSpec], seed: int, dtype: torch.dt
             for name, rows in zip(spec.merged_from, spec.merged_rows):
                 t[row: row + rows] = _draw(name, (rows, *spec.shape[1:]), spec.init, spec.std, seed, device).to(dtype)
                 row += rows
-            out[spec.name] = t
         else:
-            out[spec.name] = _draw(spec.name, spec.shape, spec.init, spec.std, seed, device).to(dtype)
+            t = _draw(spec.name, spec.shape, spec.init, spec.std, seed, device).to(dtype)
+        out[spec.name] = spec.taken(t)
     return out
 
 
