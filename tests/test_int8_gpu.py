@@ -789,3 +789,24 @@ def test_portions_without_memory_for_scratch(dtype, monkeypatch) -> None:
     out = attend(q, cache, 16, tables, ctx, 0, 0.09)
     assert len(lost) == 1 and lost[0] >= 3000 * 2 * 2 * 128 * q.element_size()
     attention_holds(q, cache, 16, tables, ctx, 0, out, 0.09)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d,page", [(8, 2, 128, 16), (4, 4, 64, 8), (12, 2, 96, 16), (6, 2, 80, 16), (3, 1, 36, 5)])
+@pytest.mark.parametrize("new,n", [(1, 1), (1, 300), (1, 3000), (5, 90), (7, 7)])
+def test_attention_where_every_score_is_far_below_zero(dtype, hq, hkv, d, page, new, n) -> None:
+    """Scores of -1e32, far enough apart that the best key takes all: its values come out, as for any other scores. Head by head
+    all keys' elements are of one sign and the queries of the other; a key's codes are its place, so the first one scores best."""
+    ctx = step_of([new], [n], dtype)
+    tables, pages = tables_for([n], page)
+    cache = cache_of(pages, hkv, page, d)
+    cache[0][:] = 0
+    cache[2][:] = 1.0
+    place = torch.arange(n, device="cuda")
+    cache[0][tables[0].long()[place // page], :, place % page] = torch.clamp(place + 1, max=127).to(torch.int8)[:, None, None]
+    q = torch.full((new, hq, d), -1e30, dtype=dtype, device="cuda")
+    out = attend(q, cache, page, tables, ctx, 0, 1.0).view(new, hkv, hq // hkv, d)
+    first = (cache[1][int(tables[0, 0]), :, 0].double() * cache[3][int(tables[0, 0])].double()[:, None])[None, :, None]
+    step = 2.0 ** -20 if dtype == torch.float32 else 2.0 ** -7
+    assert bool(((out.double() - first).abs() <= step * first.abs()).all())

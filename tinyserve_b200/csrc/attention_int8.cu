@@ -333,7 +333,7 @@ __device__ __forceinline__ void take_codes(uint32_t (&w)[BYTES / 4], const unsig
 // Queries of 32 bits: their elements as the sum of three fp16 numbers (exactly, but for what lies below 2^-39 of the row's
 // largest), the codes without their offset, the weights as the sum of two (22 bits): three products for one and two for one, eight
 // rows a CTA at most.
-constexpr float AI_FLOOR = -1e30f;            // the running maximum of nothing: finite, so that hidden places need no care
+constexpr float AI_FLOOR = -3e38f;            // the running maximum of nothing: finite, so that hidden places need no care, and below all scores
 constexpr float AI_LIFT = 6.f;
 template <int D> constexpr int AI_PITCH = D <= 64 ? 64 : 128;                   // of a row in the ring
 constexpr int AI_STAGES = 3, AI_TILES = 2, AI_KEYS = 16 * AI_TILES;
