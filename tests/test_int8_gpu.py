@@ -810,3 +810,30 @@ def test_attention_where_every_score_is_far_below_zero(dtype, hq, hkv, d, page, 
     first = (cache[1][int(tables[0, 0]), :, 0].double() * cache[3][int(tables[0, 0])].double()[:, None])[None, :, None]
     step = 2.0 ** -20 if dtype == torch.float32 else 2.0 ** -7
     assert bool(((out.double() - first).abs() <= step * first.abs()).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hkv,d,page", [(8, 128, 16), (5, 36, 16), (3, 50, 7)])
+def test_codes_of_the_cache_are_quotients_rounded_once(dtype, hkv, d, page) -> None:
+    """A value over its scale, correctly rounded, to the nearest code: many bf16 values lie half a step between two (half of the
+    largest is 63.5 steps), where one rounding more falls to the other side. The same for what a page held, in its new scale."""
+    new, lens = [90 * page] + [1] * 60, [90 * page] + [page + 3] * 60
+    ctx = step_of(new, lens, dtype)
+    tables, pages = tables_for(lens, page)
+    cache = cache_of(pages, hkv, page, d)
+    k, v = rnd(ctx.num_tokens, hkv, d, dtype=dtype, seed=1), rnd(ctx.num_tokens, hkv, d, dtype=dtype, seed=2, scale=0.3)
+    before = [x.clone() for x in cache]
+    ops.kv_write_int8(k, v, *cache, page, tables, ctx)
+    seen = 0
+    for rows, codes, scales, had, had_scale in ((k, cache[0], cache[2], before[0], before[2]), (v, cache[1], cache[3], before[1], before[3])):
+        for r, block, lo, hi, shift in ref.touched(ctx, page):
+            p, held = int(tables[r, block]), lo - block * page
+            s = scales[p][:, None, None]
+            fresh = rows[lo + shift: hi + shift].float().transpose(0, 1)
+            assert torch.equal(codes[p, :, held: held + hi - lo], torch.round(fresh / s).to(torch.int8))
+            kept, grew = had[p, :, :held], (scales[p] > had_scale[p])[:, None, None]
+            again = torch.round(kept.float() * had_scale[p][:, None, None] / s).to(torch.int8)
+            assert torch.equal(codes[p, :, :held], torch.where(grew, again, kept))
+            seen += int(grew.sum()) if held else 0
+    assert seen > 20

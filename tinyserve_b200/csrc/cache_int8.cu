@@ -62,7 +62,15 @@ __global__ void __launch_bounds__(128) kv_write_int8_kernel(const T* __restrict_
   const float need = int8_scale(m);
   const bool lost = !(need < INFINITY) || !(before < INFINITY);        // an infinity or a NaN, now or earlier
   const float scale = lost ? __uint_as_float(INT8_NAN_BITS) : fmaxf(before, need);
-  const float inverse = lost || scale == 0.f ? 0.f : 1.f / scale, ratio = before * inverse;
+  const float inverse = lost || scale == 0.f ? 0.f : 1.f / scale;
+  // The quotient by the scale, rounded once: half of the largest of values with 8-bit mantissas is 63.5 steps, and products with the
+  // rounded reciprocal alone fall to its other side more often. One correction by the remainder, which fma leaves whole (Markstein,
+  // IBM J. Res. Dev. 34, 1990); portions of 3 x 683 tokens, the product alone / so / divided: 6.8 / 7.4 / 8.7 us. (A NaN becomes
+  // the code 0.)
+  auto code_of = [&](float v) {
+    const float q = v * inverse;
+    return (int8_t)__float2int_rn(fmaf(fmaf(-q, scale, v), inverse, q));
+  };
   if (threadIdx.x == 0) *scale_at = scale;
   if (lost || scale > before) {
     for (int i = threadIdx.x * VEC; i < held * dim; i += 128 * VEC) {
@@ -70,7 +78,7 @@ __global__ void __launch_bounds__(128) kv_write_int8_kernel(const T* __restrict_
       if constexpr (VEC == 4) *reinterpret_cast<int*>(c) = *reinterpret_cast<const int*>(codes + i);
       else c[0] = codes[i];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) c[e] = (int8_t)(lost ? 0 : int8_code((float)c[e], ratio));
+      for (int e = 0; e < VEC; ++e) c[e] = lost ? (int8_t)0 : code_of((float)c[e] * before);
       if constexpr (VEC == 4) *reinterpret_cast<int*>(codes + i) = *reinterpret_cast<const int*>(c);
       else codes[i] = c[0];
     }
@@ -80,7 +88,7 @@ __global__ void __launch_bounds__(128) kv_write_int8_kernel(const T* __restrict_
     load(i, f);
     alignas(4) int8_t c[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) c[e] = (int8_t)int8_code(f[e], inverse);
+    for (int e = 0; e < VEC; ++e) c[e] = code_of(f[e]);
     if constexpr (VEC == 4) *reinterpret_cast<int*>(codes + held * dim + i * 4) = *reinterpret_cast<const int*>(c);
     else codes[held * dim + i] = c[0];
   }
