@@ -837,3 +837,19 @@ def test_codes_of_the_cache_are_quotients_rounded_once(dtype, hkv, d, page) -> N
             assert torch.equal(codes[p, :, :held], torch.where(grew, again, kept))
             seen += int(grew.sum()) if held else 0
     assert seen > 20
+
+
+@gpu
+def test_portions_some_at_a_time_with_indices_checked(monkeypatch) -> None:
+    """The check of block tables (``TINYSERVE_B200_CHECK_INDICES``) looks at all rows of the table of values, of which a run of
+    requests fills its own: the others hold pages that are there, whatever the memory held before."""
+    new, lens = [200, 1, 100, 300], [320, 30, 640, 944]
+    ctx, tables, cache, q = portions_case(new, lens, 8, 2, 128, 16, torch.bfloat16)
+    tables[tables >= cache[0].shape[0]] = 0
+    ctx.arena.take((1 << 20,), torch.int32).fill_(2 ** 30)
+    ctx.arena.begin_step()
+    monkeypatch.setattr(ops, "CHECK_INDICES", True)
+    monkeypatch.setattr(ops, "_int8_direct_rows", lambda *_: 0)
+    monkeypatch.setattr(ops, "INT8_PORTIONS_SCRATCH_BYTES", 60 * 2 * 2 * 16 * 128 * 2)
+    out = attend(q, cache, 16, tables, ctx, 0, 0.09)
+    attention_holds(q, cache, 16, tables, ctx, 0, out, 0.09)

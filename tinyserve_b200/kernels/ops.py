@@ -2811,6 +2811,8 @@ def _portions_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         return left + [(a, b) for a, b, _ in runs]
     k, v = (both[at: at + size].view(dt).view(pages, hkv, page_size, d) for at in (0, second))
     tables = ctx.arena.take((ctx.num_seqs, width), torch.int32)
+    if runs[0][1] - runs[0][0] < ctx.num_prefill:
+        tables.zero_()          # a run fills the rows of its own requests: the others are to hold a page that is there
     for a, b, _ in runs:
         part, lo, hi = _PortionsOnly(ctx), 0, ctx.num_seqs
         if b - a < ctx.num_prefill:
