@@ -12,10 +12,13 @@
 
 namespace ts {
 
-// One CTA for each (page that gets tokens, key/value head, keys or values): the only one that touches them, so there are no
-// atomics and no order to depend on. A thread takes VEC neighbouring elements of a row at a time (the new rows are read twice, the
-// second time from L1). Bound by latency: the lengths, the table, the rows and the old scale, then the codes; a token each for 64
-// requests with 8 heads of 128 takes 3.1 us, three portions of 683 tokens 7.5 us (12.7 MB).
+// One CTA for each (page that gets tokens, key/value head, keys or values). A page belongs to one request of a step, so it is the only
+// one that touches them, and there are no atomics and no order to depend on. (The exception is the page of the rows that fill up a
+// recorded step: their CTAs write over one another there, and what they leave is read by those rows alone, whose results nobody
+// reads. Each is a request of one token, so none reads a code or a scale that another writes.) A thread takes VEC neighbouring
+// elements of a row at a time (the new rows are read twice, the second time from L1). Bound by latency: the lengths, the table, the
+// rows and the old scale, then the codes; a token each for 64 requests with 8 heads of 128 takes 3.0 us, three portions of 683 tokens
+// 7.4 us with their rows in L2 and 9.8 from memory (12.7 MB).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(128) kv_write_int8_kernel(const T* __restrict__ k, const T* __restrict__ v, int8_t* __restrict__ k_cache,
                                                             int8_t* __restrict__ v_cache, float* __restrict__ k_scales,

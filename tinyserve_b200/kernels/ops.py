@@ -2577,8 +2577,8 @@ def int8_weight(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     codes = torch.empty((w.shape[0], int8_width(w.shape[1])), dtype=torch.int8, device=w.device)
     scales = torch.empty(w.shape[0], dtype=torch.float32, device=w.device)
     act_mul_int8(w, codes, scales, "none")
-    # A product asks for its first weights in front of its wait for this library's earlier kernels; behind a kernel of another
-    # library, which it always waits for, they are there.
+    # A product asks for its first weights in front of its wait for this library's earlier kernels, several of which may still run
+    # then; behind a kernel of another library, which it always waits for, they are there.
     return codes, scales.clone()
 
 
@@ -2633,7 +2633,8 @@ def int8_product_form(m: int, n: int, k: int) -> tuple[int, int, int]:
 def gemm_int8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor) -> None:
     """``out[m, n] = dt((sum_k x[m, k] w[n, k]) * (x_scales[m] * w_scales[n]))``: ``x`` ``[M, K]`` and ``w`` ``[N, K]`` int8, K a multiple
     of 16 (rows padded with zeros, :func:`int8_width`) up to 131,072; the sum is exact in 32-bit integers. ``w`` is a weight: no
-    kernel of this library that was launched just before may be writing it (:func:`int8_weight`)."""
+    kernel of this library may be writing it that was launched since the stream's last other work (a kernel of torch, a copy): a product
+    may begin to read it while several of the kernels in front of it still run (:func:`int8_weight` leaves such work behind itself)."""
     m, k = x.shape
     n, kw = w.shape
     if kw != k or out.shape != (m, n) or x_scales.shape != (m,) or w_scales.shape != (n,):
