@@ -228,7 +228,12 @@ __global__ void __launch_bounds__(128 * ACCS) gemm_int8_rows_kernel(const __grid
       uint32_t parity = 0;
       for (int i = 0; i < num_kb && ok; ++i) {
         ok = mbar_wait(&full_bar[s], parity);
-        if (!ok) { *(volatile int*)&failed = 1; break; }
+        if (!ok) {
+          *(volatile int*)&failed = 1;
+          // the copies of this round of the ring may still be on their way, and their thread gone: stay for them, once more with the limit
+          for (int j = i; j < num_kb && j < i + stages; ++j) mbar_wait(&full_bar[j % stages], (j / stages) & 1);
+          break;
+        }
         tc_fence_after();
         const uint32_t a_addr = smem_u32(ring + (size_t)s * stage);
         const uint64_t bdesc = sw128_desc(a_addr + w_bytes);
@@ -498,6 +503,9 @@ __global__ void __launch_bounds__(MR_THREADS) gemm_int8_pair_kernel(const __grid
       // the even CTA's last commits also arrive at this CTA's barriers: stay until they have
       for (int j = it > STAGES ? it - STAGES : 0; j < it && !failed; ++j)
         if (!mbar_wait(&empty_bar[j % STAGES], (j / STAGES) & 1)) failed = 1;
+      // after a failure: copies in flight may still land in either CTA's shared memory (the even one's barriers count both's)
+      if (failed && leader)
+        for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(&full_bar[j % STAGES], (j / STAGES) & 1);
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (one lane of the even CTA)
