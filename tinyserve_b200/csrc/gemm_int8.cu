@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(128 * ACCS) gemm_int8_rows_kernel(const __grid
         ok = mbar_wait(&full_bar[s], parity);
         if (!ok) {
           *(volatile int*)&failed = 1;
-          // the copies of this round of the ring may still be on their way, and their thread gone: stay for them, once more with the limit
+          // the copies of this turn of the ring may still be on their way, and their thread gone: stay for them, once more with the limit
           for (int j = i; j < num_kb && j < i + stages; ++j) mbar_wait(&full_bar[j % stages], (j / stages) & 1);
           break;
         }
